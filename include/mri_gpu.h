@@ -338,7 +338,11 @@ MRI_API int mri_llama_attention_fallbacks(const mri_llama* m, size_t* count);
  * head_dim is 32, 64, 96 or 128 and capacity a positive multiple of 64, else
  * MRI_ERR_INVALID_SHAPE; null or misaligned buffers -> MRI_ERR_INVALID_ARGUMENT.
  * Calls are asynchronous on the context's stream.  Lengths and positions are
- * device int32 values, so a captured graph can replay with new ones. */
+ * device int32 values, so a captured graph can replay with new ones.  A first
+ * call of the same sizes has to size the context's scratch before the capture
+ * (MRI_ERR_CUDA while capturing otherwise); later, larger calls leave the graph
+ * its scratch.  Replays share the context's scratch and counters with its other
+ * calls, so they must be ordered with those, and end before the context does. */
 typedef struct mri_kv4_cache {
   uint8_t* k;
   uint8_t* v;

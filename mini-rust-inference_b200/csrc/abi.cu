@@ -60,14 +60,39 @@ int enter(mri_ctx* ctx) {
 
 int check_k(const char* fn, size_t m, size_t k, size_t k_w);
 
-// Scratch is one growing device buffer per context, carved by the callers.
+// Whether the context's stream is being captured into a CUDA graph.
+bool capturing(mri_ctx* ctx) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &status) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream while another one is captured: launches on it fail
+    return false;
+  }
+  return status != cudaStreamCaptureStatusNone;
+}
+
+// Scratch is one growing device buffer per context, carved by the callers.  A
+// buffer whose address a captured launch holds is not freed before the context.
 int ensure_scratch(mri_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return MRI_OK;
+  const bool captured = (!ctx->scratch_captured || bytes > ctx->scratch_bytes) && capturing(ctx);
+  if (bytes <= ctx->scratch_bytes) {
+    ctx->scratch_captured |= captured;
+    return MRI_OK;
+  }
+  if (captured)
+    return fail(MRI_ERR_CUDA,
+                "the context's scratch (%zu bytes) cannot grow to %zu while its stream is captured; make the call once "
+                "before the capture",
+                ctx->scratch_bytes, bytes);
   if (ctx->scratch) {
-    MRI_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-    MRI_CUDA_TRY(cudaFree(ctx->scratch));
+    if (ctx->scratch_captured) {
+      ctx->scratch_kept.push_back(ctx->scratch);
+    } else {
+      MRI_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+      MRI_CUDA_TRY(cudaFree(ctx->scratch));
+    }
     ctx->scratch = nullptr;
     ctx->scratch_bytes = 0;
+    ctx->scratch_captured = false;
   }
   const size_t sz = std::max<size_t>(bytes, 1 << 20);
   MRI_CUDA_TRY(cudaMalloc(&ctx->scratch, sz));
@@ -506,6 +531,7 @@ int mri_ctx_destroy(mri_ctx* ctx) {
   use_device(ctx->device);
   cudaStreamSynchronize(ctx->stream);
   if (ctx->scratch) cudaFree(ctx->scratch);
+  for (uint8_t* p : ctx->scratch_kept) cudaFree(p);
   if (ctx->h_status) cudaFreeHost(ctx->h_status);
   if (ctx->d_sync) cudaFree(ctx->d_sync);
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);

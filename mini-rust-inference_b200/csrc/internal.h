@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <vector>
 
 struct mri_ctx;
 struct mri_qmatrix;
@@ -244,9 +245,10 @@ int matmul_int8_gather(struct ::mri_ctx* ctx, const float* x, size_t m, size_t k
 bool matmul_int8_epilogue_supported(const struct ::mri_ctx* ctx, size_t m,
                                     const struct ::mri_qmatrix* w);
 
-// Grows the context scratch to at least `bytes` (synchronizes the stream
-// when it reallocates).  Callers that capture CUDA graphs reserve their
-// maximum first: a captured launch keeps the scratch address it saw.
+// Grows the context scratch to at least `bytes`: waits for the stream and frees
+// the old buffer, or keeps it until the context ends if a call that was captured
+// into a CUDA graph was given it, since the graph's launches hold its address.
+// Cannot grow while the stream is being captured: a first call sizes the scratch.
 int ctx_reserve_scratch(struct ::mri_ctx* ctx, size_t bytes);
 // Scratch bytes an INT8 product with per-tensor quantization of an [m, k]
 // input needs.
@@ -338,6 +340,8 @@ struct mri_ctx {
   unsigned kv4_evict_ready = 0;
   uint8_t* scratch = nullptr;
   size_t scratch_bytes = 0;
+  bool scratch_captured = false;       // a captured launch holds the address of `scratch`
+  std::vector<uint8_t*> scratch_kept;  // outgrown buffers that captured launches hold
   mri::LaunchStats ls;
 };
 
