@@ -389,9 +389,11 @@ MRI_API int mri_kv4_attention(mri_ctx* ctx, const mri_kv4_cache* cache, const fl
  * new_lens[b] = min(lens[b], budget); kept[b][head][budget] (nullable) receives
  * the rows' old positions, -1 past new_lens[b]; rows [new_lens[b], budget) of
  * dst become 0.  dst: same batch, heads and head_dim (else
- * MRI_ERR_SHAPE_MISMATCH), capacity >= budget, other buffers than src's.
+ * MRI_ERR_SHAPE_MISMATCH), capacity >= budget.
  * budget == 0, budget > dst->capacity or recent > budget ->
- * MRI_ERR_INVALID_SHAPE; shared buffers -> MRI_ERR_INVALID_ARGUMENT. */
+ * MRI_ERR_INVALID_SHAPE.  Outputs (dst's buffers, new_lens, kept) that overlap an
+ * input or one another -> MRI_ERR_INVALID_ARGUMENT; new_lens_dev cannot be
+ * lens_dev, which blocks still read when others have written. */
 MRI_API int mri_kv4_evict(mri_ctx* ctx, const mri_kv4_cache* src, const int32_t* lens_dev,
                           const mri_kv4_cache* dst, size_t budget, size_t recent,
                           int32_t* new_lens_dev, int32_t* kept_dev);

@@ -225,6 +225,15 @@ int matmul_int8_fused(struct ::mri_ctx* ctx, const float* x, size_t m, size_t k,
                       const EpiArgs* epi = nullptr, int pre_stages = -1);
 // Records the calling thread's last error (mri_last_error) and returns code.
 int set_error(int code, const char* fmt, ...);
+// Whether [p, p + bytes) meets one of `rows` runs of `width` bytes, `pitch` bytes apart
+// from q on.
+inline bool overlaps(const void* p, size_t bytes, const void* q, size_t width, size_t rows = 1, size_t pitch = 0) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  if (!p || !q || bytes == 0 || width == 0 || rows == 0 || a + bytes <= b) return false;
+  // The first run that ends after a.
+  const size_t r = a < b + width || rows == 1 ? 0 : (a - b - width) / pitch + 1;
+  return r < rows && a < b + r * pitch + width && b + r * pitch < a + bytes;
+}
 // Start of an entry point outside abi.cu: null check, clears the last error,
 // selects the context's device.
 int enter_ctx(struct ::mri_ctx* ctx);

@@ -1917,6 +1917,18 @@ int check_tokens(const char* fn, size_t n_tokens, size_t rows_each, size_t batch
   return MRI_OK;
 }
 
+// A buffer that a call reads or writes.
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+// The five buffers of a cache, to to[0..4].
+void spans_of(const Cache& c, Span* to) {
+  const size_t rows = static_cast<size_t>(c.batch) * c.heads * c.cap, nb = c.nb;
+  const Span all[5] = {{c.k, rows * 16 * nb}, {c.v, rows * 16 * nb}, {c.ks, rows * 2 * nb}, {c.vs, rows * 2 * nb}, {c.weight, rows * 4}};
+  std::copy(all, all + 5, to);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int NB>
@@ -2055,11 +2067,24 @@ int mri_kv4_evict(mri_ctx* ctx, const mri_kv4_cache* src, const int32_t* lens_de
                           budget, recent, d.cap);
   if (s.batch == 0) return MRI_OK;
   if (!lens_dev || !new_lens_dev) return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_kv4_evict: null pointer");
-  if (s.k == d.k || s.v == d.v || s.ks == d.ks || s.vs == d.vs || s.weight == d.weight)
-    return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_kv4_evict: source and destination share a buffer");
   const size_t rows = static_cast<size_t>(s.batch) * s.heads * budget;
   if (rows > (size_t{1} << 31) - 1)
     return mri::set_error(MRI_ERR_INVALID_SHAPE, "mri_kv4_evict: %zu rows are too many for one call", rows);
+  // Blocks write while others still read: no output may lie in an input or in another output.
+  const size_t lens_bytes = static_cast<size_t>(s.batch) * sizeof(int32_t);
+  Span reads[6], writes[7];
+  spans_of(s, reads);
+  reads[5] = {lens_dev, lens_bytes};
+  spans_of(d, writes);
+  writes[5] = {new_lens_dev, lens_bytes};
+  writes[6] = {kept_dev, rows * sizeof(int32_t)};
+  for (int i = 0; i < 7; ++i) {
+    bool shared = false;
+    for (const Span& r : reads) shared |= mri::overlaps(writes[i].p, writes[i].bytes, r.p, r.bytes);
+    for (int j = 0; j < i; ++j) shared |= mri::overlaps(writes[i].p, writes[i].bytes, writes[j].p, writes[j].bytes);
+    if (shared)
+      return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_kv4_evict: an output buffer overlaps an input or another output");
+  }
   if (!kept_dev) {
     if (int rc = mri::ctx_reserve_scratch(ctx, rows * sizeof(int32_t))) return rc;
     kept_dev = reinterpret_cast<int32_t*>(ctx->scratch);
