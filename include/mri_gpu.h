@@ -377,7 +377,10 @@ MRI_API int mri_kv4_read(mri_ctx* ctx, const mri_kv4_cache* cache, const int32_t
  * n_kv_heads -> MRI_ERR_INVALID_SHAPE, ld < n_heads * head_dim ->
  * MRI_ERR_SHAPE_MISMATCH.
  * track != 0: each row's softmax weights, summed over the tokens and query
- * heads that read it, are added to cache->weight. */
+ * heads that read it, are added to cache->weight.
+ * out_dev may be q_dev where ld = n_heads * head_dim and track == 0; any other
+ * overlap of it with an input (or of the tracked weights with the queries or
+ * lengths) -> MRI_ERR_INVALID_ARGUMENT. */
 MRI_API int mri_kv4_attention(mri_ctx* ctx, const mri_kv4_cache* cache, const float* q_dev, size_t ld,
                               size_t n_tokens, size_t n_heads, const int32_t* lens_dev, float scale,
                               int track, float* out_dev);

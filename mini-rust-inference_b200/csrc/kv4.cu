@@ -2034,6 +2034,22 @@ int mri_kv4_attention(mri_ctx* ctx, const mri_kv4_cache* cache, const float* q_d
   if (rows == 0) return MRI_OK;
   if (!q_dev || !lens_dev || !out_dev)
     return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_kv4_attention: null pointer");
+  // A unit's outputs are the places of its own queries, and are written when all of its
+  // blocks have those in registers, so out may be q itself.  Not in tracked calls, whose
+  // second pass reads the queries again.
+  const size_t tokens = static_cast<size_t>(c.batch) * n_tokens, row_bytes = n_heads * c.hd * sizeof(float);
+  const bool in_place = out_dev == q_dev && ld == n_heads * c.hd && !track;
+  const Span tracked{track ? c.weight : nullptr, static_cast<size_t>(c.batch) * c.heads * c.cap * sizeof(float)};
+  Span reads[6];
+  spans_of(c, reads);
+  reads[5] = {lens_dev, static_cast<size_t>(c.batch) * sizeof(int32_t)};
+  bool shared = !in_place && mri::overlaps(out_dev, tokens * row_bytes, q_dev, row_bytes, tokens, ld * sizeof(float));
+  shared |= mri::overlaps(tracked.p, tracked.bytes, q_dev, row_bytes, tokens, ld * sizeof(float));
+  shared |= mri::overlaps(tracked.p, tracked.bytes, lens_dev, reads[5].bytes);
+  for (const Span& r : reads) shared |= mri::overlaps(out_dev, tokens * row_bytes, r.p, r.bytes);
+  if (shared)
+    return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_kv4_attention: an output buffer overlaps an input%s",
+                          track ? " (a tracked call reads the queries again after its outputs)" : "");
   AttnArgs a{};
   a.c = c;
   a.q = q_dev;
