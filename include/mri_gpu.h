@@ -423,7 +423,9 @@ MRI_API int mri_kv4_evict(mri_ctx* ctx, const mri_kv4_cache* src, const int32_t*
  * accepted [batch]: n; logprobs (nullable) [batch][n_drafts + 1]: log p of each
  * token given (at temperature 1 where greedy), 0 past them.
  * n_drafts > 64, or vocab == 0 -> MRI_ERR_INVALID_SHAPE.  A temperature
- * that is negative or not finite counts as 1. */
+ * that is negative or not finite counts as 1.  Outputs that overlap an input or
+ * one another -> MRI_ERR_INVALID_ARGUMENT; tokens_dev may be draft_tokens_dev
+ * where batch == 1. */
 MRI_API int mri_verify_draft(mri_ctx* ctx, const float* target_logits_dev,
                              const int32_t* draft_tokens_dev, const float* uniforms_dev,
                              const float* races_dev, const float* draft_probs_dev,

@@ -384,6 +384,25 @@ extern "C" int mri_verify_draft(mri_ctx* ctx, const float* target_logits_dev, co
   if (!target_logits_dev || !races_dev || !tokens_dev || !accepted_dev ||
       (n_drafts && (!draft_tokens_dev || !uniforms_dev)))
     return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_verify_draft: null pointer");
+  // A sequence's outputs are written while others still read their inputs; only a lone
+  // sequence's tokens may take the place of its drafts (its blocks have read them).
+  struct Span {
+    const void* p;
+    size_t bytes;
+  };
+  const size_t drafts = batch * n_drafts * 4, given = batch * (n_drafts + 1) * 4, row = batch * vocab * 4;
+  const Span reads[] = {{target_logits_dev, row * (n_drafts + 1)}, {draft_probs_dev, row * n_drafts}, {races_dev, row},
+                        {uniforms_dev, drafts}, {temperature_dev, batch * 4}, {draft_tokens_dev, drafts}};
+  const Span writes[] = {{tokens_dev, given}, {accepted_dev, batch * 4}, {logprobs_dev, given}};
+  for (const Span& w : writes) {
+    bool shared = false;
+    for (const Span& r : reads)
+      if (!(batch == 1 && r.p == draft_tokens_dev && w.p == tokens_dev && r.p == w.p))
+        shared |= mri::overlaps(w.p, w.bytes, r.p, r.bytes);
+    for (const Span* o = writes; o != &w; ++o) shared |= mri::overlaps(w.p, w.bytes, o->p, o->bytes);
+    if (shared)
+      return mri::set_error(MRI_ERR_INVALID_ARGUMENT, "mri_verify_draft: an output overlaps an input or another output");
+  }
   // Blocks of a sequence: as many as the GPU still takes at once, each with at least
   // 2048 values of a row.  48 sequences of 8 rows of 32000: 21 us with 16 values a
   // thread, 31 with 8; one of 5 rows: 9.0 and 8.2; 16 of 4 rows of 50001: 17 us in

@@ -257,3 +257,39 @@ def test_refusals(mri, gpu_ctx):
     assert lib.mri_verify_draft(h, None, p, p, p, None, None, 1, 1, 4, p, p, None) == 6
     assert lib.mri_verify_draft(h, p, None, p, p, None, None, 1, 1, 4, p, p, None) == 6
     assert lib.mri_verify_draft(h, p, p, p, p, None, None, 1, 1, 0, p, p, None) == 1
+
+
+def test_overlapping_buffers(mri, gpu_ctx):
+    """An output in an input's place is refused; a lone sequence's tokens may take its drafts' place."""
+    import torch
+    rng = np.random.default_rng(13)
+    lib, h = gpu_ctx._lib, gpu_ctx.handle
+    for b in (1, 3):
+        logits, drafts, u, e, q = (gpu(a) for a in inputs(rng, b, 2, 5000))
+        temp = torch.full((b,), 0.8, device="cuda")
+        tokens, accepted, lp = mri.verify_draft(logits, drafts, u, e, draft_probs=q, temperature=temp)
+        ins = [t.data_ptr() for t in (logits, drafts, u, e, q, temp)]
+        room = torch.zeros(b * 3, dtype=torch.int32, device="cuda")
+        room[:b * 2] = drafts.flatten()
+        outs = [torch.zeros_like(t) for t in (tokens, accepted, lp)]
+
+        def call(at=ins, out=[t.data_ptr() for t in outs]):
+            return lib.mri_verify_draft(h, *at, b, 2, 5000, *out)
+
+        torch.cuda.synchronize()
+        launches = gpu_ctx.launch_count
+        for i in range(3):
+            for other in ins + [outs[(i + 1) % 3].data_ptr()]:
+                out = [t.data_ptr() for t in outs]
+                out[i] = other
+                if not (b == 1 and i == 0 and other == ins[1]):
+                    assert call(out=out) == 6, (b, i)
+        assert call(out=[room.data_ptr() + 4] + [t.data_ptr() for t in outs[1:]], at=[ins[0], room.data_ptr()] + ins[2:]) == 6
+        in_place = dict(out=[room.data_ptr()] + [t.data_ptr() for t in outs[1:]], at=[ins[0], room.data_ptr()] + ins[2:])
+        if b > 1:
+            assert call(**in_place) == 6
+        assert gpu_ctx.launch_count == launches
+        if b == 1:
+            assert call(**in_place) == 0
+            gpu_ctx.synchronize()
+            assert torch.equal(room.view(1, 3), tokens) and torch.equal(outs[1], accepted) and torch.equal(outs[2], lp)
