@@ -1186,6 +1186,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
           next += (first - next + a.splits - 1) / a.splits * a.splits;
         }
       }
+      __syncwarp();  // lane 0's unit is read by all lanes: a shuffle alone orders no memory
       next = __shfl_sync(0xffffffffu, next, 0);
       if (next >= count) return;
       const Unit& v = ahead[wk];
