@@ -370,7 +370,9 @@ MRI_API int mri_kv4_read(mri_ctx* ctx, const mri_kv4_cache* cache, const int32_t
  * tokens' own rows included: query t sees rows [0, lens[b] - n_tokens + 1 + t).
  * A query that sees no row gets 0.  lens[b] is taken as clamped to [0,
  * capacity]; rows from lens[b] on are not used, whatever they hold.  The lengths
- * are read throughout the call: what changes them has to run after it.
+ * are read throughout the call: what changes them has to run after it.  If they
+ * change all the same the call still ends, but its results, and those of the
+ * context's later attention calls, are lost.
  * q_dev f32 [batch][n_tokens] rows of n_heads * head_dim values, ld floats
  * apart; out_dev f32 [batch][n_tokens][n_heads][head_dim].  Head h reads
  * key/value head h / (n_heads / n_kv_heads); n_heads not a positive multiple of

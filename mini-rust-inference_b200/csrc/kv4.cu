@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "kv4_walk.h"
 #include "mri_gpu.h"
 
 namespace {
@@ -421,52 +422,20 @@ struct AttnArgs {
   float* part;      // [2 * grid][n_rows][hd + 4]
   unsigned* ready;  // [grid], zero between calls
   int2* spans;      // of each unit: the first and the last block that have a part in it
+  unsigned grid;    // blocks of the first kernel
   int* status;
+  __device__ __forceinline__ int len(int b) const { return min(max(mri::ld_act(lens + b), 0), static_cast<int>(c.cap)); }
 };
 
-// A unit of work: one row group of one key/value head.  Units are numbered
-// (entry, row group, head); their stages of a.keys keys make one flat range that
-// the blocks share evenly.
-struct Unit {
-  int b, rg, h;
-  int tiles;  // places of this unit, its stages last
-  int end;    // its last stage + 1, counted from the block's first stage
-};
+using mri::kv4::Plan;
+using mri::kv4::Unit;
+using mri::kv4::next_segment;
+using mri::kv4::next_unit;
+using mri::kv4::owner_of;
+using mri::kv4::seek_stage;
+using mri::kv4::unit_tiles;
 
-__device__ __forceinline__ int entry_len(const AttnArgs& a, int b) {
-  return min(max(mri::ld_act(a.lens + b), 0), static_cast<int>(a.c.cap));
-}
-
-// What a unit counts in the range that the blocks share: the stages of its row group
-// (up to the last key its last row sees, at least one: rows that see nothing are
-// written too), after a.pad places for what a unit costs besides.
-__device__ __forceinline__ int unit_tiles(const AttnArgs& a, int b, int rg) {
-  const int last = min((rg + 1) * a.n_rows, a.rows) - 1;
-  const int seen = entry_len(a, b) - a.n_tokens + 1 + last / a.group;
-  return a.pad + max(1, (seen + a.keys - 1) / a.keys);
-}
-
-__device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
-  if (++u.h == a.c.heads) {
-    u.h = 0;
-    if (++u.rg == a.row_groups) {
-      u.rg = 0;
-      ++u.b;
-    }
-    u.tiles = u.b < a.c.batch ? unit_tiles(a, u.b, u.rg) : 0;
-  }
-  u.end += u.tiles;
-}
-
-struct Plan {
-  unsigned total, x0;     // stages of the call (below 2^32); the block's first
-  int count;              // stages of the block
-  unsigned blocks;        // blocks with a share
-  unsigned each, longer;  // a share's stages; the first `longer` blocks have one more
-  Unit first;
-};
-
-// This block's share of the flat range and the unit it begins in.
+// This block's share of the call's stages and the unit it begins in.
 // Every thread calls it; sums over (entry, row group) pairs in shared memory.
 __device__ __forceinline__ void make_plan(const AttnArgs& a, Plan* plan, unsigned* sh) {
   const unsigned threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -491,38 +460,12 @@ __device__ __forceinline__ void make_plan(const AttnArgs& a, Plan* plan, unsigne
     if (w < warp) before += sh[w];
     total += sh[w];
   }
-  const unsigned least = kMinKeys / static_cast<unsigned>(a.keys);
-  const unsigned blocks = min(gridDim.x, (total + least - 1) / least);
-  const unsigned each = total / blocks, longer = total % blocks, c = blockIdx.x;
-  const unsigned x0 = c < blocks ? c * each + min(c, longer) : total;
-  if (threadIdx.x == 0) {
-    plan->total = total;
-    plan->blocks = blocks;
-    plan->each = each;
-    plan->longer = longer;
-    plan->x0 = x0;
-    plan->count = c < blocks ? static_cast<int>(each + (c < longer)) : 0;
-  }
-  if (x0 >= before && x0 - before < mine) {
-#pragma unroll 1
-    for (unsigned p = p0; p < p1; ++p) {
-      const int b = static_cast<int>(p / groups), rg = static_cast<int>(p % groups);
-      const unsigned tiles = static_cast<unsigned>(unit_tiles(a, b, rg));
-      if (x0 - before < tiles * heads) {
-        const unsigned h = (x0 - before) / tiles;
-        plan->first = Unit{b, rg, static_cast<int>(h), static_cast<int>(tiles), static_cast<int>((h + 1) * tiles - (x0 - before))};
-        break;
-      }
-      before += tiles * heads;
-    }
-  }
+  Plan p;
+  mri::kv4::share_out(a, total, blockIdx.x, gridDim.x, kMinKeys / static_cast<unsigned>(a.keys), p);
+  if (threadIdx.x == 0) *plan = p;
   __syncthreads();
-}
-
-// The block whose share holds flat stage x.
-__device__ __forceinline__ int owner_of(const Plan& p, unsigned x) {
-  const unsigned edge = p.longer * (p.each + 1);
-  return static_cast<int>(x < edge ? x / (p.each + 1) : p.longer + (x - edge) / p.each);
+  if (p.x0 >= before && p.x0 - before < mine) mri::kv4::find_first(a, p.x0, before, p0, p1, plan->first);
+  __syncthreads();
 }
 
 // One row tile's queries as A fragments: high parts in rows 0..7, low in
@@ -1177,15 +1120,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
     if (next >= stop) {
       if (next >= count) return;
       __syncwarp();
-      if (lane == 0) {
-        Unit& v = ahead[wk];
-        while (next < count) {
-          while (next >= v.end) next_unit(a, v);
-          const int first = v.end - v.tiles + a.pad;
-          if (next >= first) break;
-          next += (first - next + a.splits - 1) / a.splits * a.splits;
-        }
-      }
+      if (lane == 0) next = seek_stage(a, ahead[wk], next, count);
       __syncwarp();  // lane 0's unit is read by all lanes: a shuffle alone orders no memory
       next = __shfl_sync(0xffffffffu, next, 0);
       if (next >= count) return;
@@ -1217,19 +1152,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
   }
 
   Unit u = plan.first;
-  int x = 0, s = 0, used = 0;  // s: the ring's next slot
+  int x = 0, unit_begin, seg_end;  // the unit's stages of this block: [x, seg_end)
+  int s = 0, used = 0;             // s: the ring's next slot
   unsigned parity = 0;
-  while (x < count) {
-    // The unit's stages of this block: [x, seg_end).
-    const int seg_end = min(u.end, count), unit_begin = u.end - u.tiles + a.pad;
-    x = max(x, unit_begin);
-    if (x >= seg_end) {
-      x = seg_end;
-      next_unit(a, u);
-      continue;
-    }
+  while (next_segment(a, u, x, count, unit_begin, seg_end)) {
     const int row = u.rg * n_rows + wr * (8 * R) + g;
-    const int len = entry_len(a, u.b);
+    const int len = a.len(u.b);
     WarpQueries<NB, R> q;
     q.load(a, u.b, u.h, row, queries_sh);
     RowState<NB, R> r;
@@ -1360,7 +1288,8 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(AttnArgs a, un
   const unsigned unit = blockIdx.x / blocks_per_unit, pair = unit / static_cast<unsigned>(a.c.heads);
   const int2 span = mri::ld_act(a.spans + unit);
   const int c0 = span.x, c1 = span.y;
-  if (c0 == c1) return;
+  // One block's, or (lengths that changed) no block began the unit.
+  if (static_cast<unsigned>(c0) >= static_cast<unsigned>(c1) || static_cast<unsigned>(c1) >= a.grid) return;
   const unsigned groups = static_cast<unsigned>(a.row_groups);
   const Unit u{static_cast<int>(pair / groups), static_cast<int>(pair % groups), static_cast<int>(unit % static_cast<unsigned>(a.c.heads)), 0, 0};
   const int i0 = static_cast<int>(blockIdx.x % blocks_per_unit) * (kMergeThreads * kMergeItems);
@@ -1427,7 +1356,7 @@ __global__ void __launch_bounds__(kTrackWarps * 32) kv4_track_few_kernel(AttnArg
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const unsigned head = blockIdx.x / blocks_per_head;
   const int h = static_cast<int>(head % a.c.heads), b = static_cast<int>(head / a.c.heads);
-  const int len = entry_len(a, b);
+  const int len = a.len(b);
   const int64_t first = (static_cast<int64_t>(blockIdx.x % blocks_per_head) * kTrackWarps + warp) * kTrackRun;
   if (first >= len) return;
   QueryTile<NB> q;
@@ -1471,7 +1400,7 @@ __global__ void __launch_bounds__(kTrackWarps * 32) kv4_fragments_kernel(AttnArg
   QueryTile<NB> q;
   load_queries<NB>(a, entry, h, row, q);
   int end;
-  const float2 st = row_stats(a, entry, h, row, entry_len(a, entry), &end);
+  const float2 st = row_stats(a, entry, h, row, a.len(entry), &end);
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1489,7 +1418,7 @@ __global__ void __launch_bounds__(kTrackWarps * 32) kv4_track_many_kernel(AttnAr
   const unsigned head = blockIdx.x / blocks_per_head;
   const int h = static_cast<int>(head % a.c.heads), b = static_cast<int>(head / a.c.heads);
   const int64_t first = (static_cast<int64_t>(blockIdx.x % blocks_per_head) * kTrackWarps + warp) * 32;
-  const int len = entry_len(a, b);
+  const int len = a.len(b);
   if (first >= len) return;
   const int key0 = static_cast<int>(first);
   const size_t row0 = a.c.row(b, h, static_cast<size_t>(key0));
@@ -1607,6 +1536,7 @@ int launch_attention(mri_ctx* ctx, AttnArgs a, bool track) {
   a.stats = track ? reinterpret_cast<float2*>(ctx->scratch + part_bytes) : nullptr;
   a.spans = reinterpret_cast<int2*>(ctx->scratch + part_bytes + stat_bytes);
   a.ready = ctx->d_sync + mri_ctx::kSyncAttn;
+  a.grid = grid;
   a.status = ctx->d_status;
   KV4_CUDA_TRY(launch(ctx, kernel, grid, threads, smem, a));
   if (!few) {
