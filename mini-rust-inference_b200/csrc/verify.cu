@@ -64,11 +64,13 @@ __device__ __forceinline__ void pdl_enter() {
 // NaN -> -inf, +inf -> the largest finite value (fmaxf drops a NaN).
 __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 
-// 1 / temperature; greedy entries (temperature 0) are scored at 1.
+// 1 / temperature; greedy entries (temperature 0) are scored at 1.  At most 2^127, so that
+// it and its product with log2 e are finite: subnormal temperatures below 2^-127 count as
+// that, at which logits 2^-119 apart are past exp's range already.
 __device__ __forceinline__ float inverse_temperature(const Args& a, int b, bool* greedy) {
   const float t = a.temperature ? mri::ld_act(a.temperature + b) : 1.0f;
   *greedy = t == 0.0f;
-  return t > 0.0f && !isinf(t) ? __fdiv_rn(1.0f, t) : 1.0f;
+  return t > 0.0f && !isinf(t) ? fminf(__fdiv_rn(1.0f, t), 1.7014118346046923e38f) : 1.0f;
 }
 
 // A value with its index; the larger value wins, of equal ones the lower index.

@@ -192,6 +192,25 @@ def test_odd_temperatures(mri, gpu_ctx):
     check(mri, logits, drafts, u, e, None, np.array([-1, np.nan, np.inf, 1e-3, 50], np.float32))
 
 
+def test_subnormal_temperatures(mri, gpu_ctx):
+    """1 / t, or its product with log2 e, is past float32: the draws are those of the largest logits."""
+    rng = np.random.default_rng(12)
+    logits, drafts, u, e, _ = inputs(rng, 6, 2, 100, sampled=False)
+    drafts[::2] = logits[::2, :2].argmax(-1)
+    temp = np.array([4.1e-39, 2.9e-39, 1e-39, 1e-42, 1.4e-45, 1.2e-38], np.float32)
+    accepted = check(mri, logits, drafts, u, e, None, temp)
+    assert (accepted[::2] == 2).all()
+    # Equal largest logits share the probability.
+    logits[:, :, 17] = logits[:, :, 61] = 9.0
+    accepted = check(mri, logits, np.full_like(drafts, 61), np.full_like(u, 0.49), e, None, temp)
+    assert (accepted == 2).sum() >= 4
+    t, n, lp = (x.cpu().numpy() for x in mri.verify_draft(gpu(logits), gpu(np.full_like(drafts, 61)), gpu(np.full_like(u, 0.49)),
+                                                          gpu(e), temperature=gpu(temp)))
+    for i in np.flatnonzero(logits.max((1, 2)) == 9):
+        assert n[i] == 2 and t[i].tolist() == [61, 61, 17 if e[i, 17] <= e[i, 61] else 61]
+        assert np.abs(lp[i] + np.log(2)).max() <= 1e-6
+
+
 def test_draws_follow_the_target(mri, gpu_ctx):
     """Speculative sampling leaves the target's distribution: the first token
     over 40000 trials against p (chi-square, 9 degrees of freedom, below 33.7:
