@@ -280,10 +280,16 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, const int32
 //   O += P V: the scales belong to keys, the summed index, so they go into
 //   P: per block, A = f16 high and low parts of P * scale, B = the codes.
 //
-// P is taken relative to a reference that keeps P * scale in f16's range: the
-// row's running maximum and the largest value scale seen, moved (and the sums
-// rescaled) only when a score passes the old maximum by 2^8 or a scale passes
-// the old largest.  exp2 of log2-scaled scores; sums and scores in f32.
+// An f16 pair holds P * scale to 22 bits from 2^-2 up, and to 2^-25 below.  P is taken
+// relative to a reference below the row's running maximum, moved (and the sums rescaled)
+// only when a score passes the old maximum by 2^kRise; value scales by a factor of their
+// block (the same 32 columns) that brings the largest one the warp has seen below
+// 2^kTop, moved when one passes that.  So a block of small values is as exact as one of
+// large ones.  Within a block a key has its 22 bits down to 2^-11 of the row's
+// largest P times the block's largest scale, whoever's that is, and a bit less with every
+// factor of 2 from there: keys beside one of 2^11 times their values, in a row in
+// which that one counts for nothing, are where f32 products would hold more.
+// exp2 of log2-scaled scores; sums and scores in f32.
 
 constexpr int kStep = 32;        // keys that are scored together; a ring's stage is one or two steps
 constexpr int kMaxWarps = 4;     // of a block: rings of their own (up to 8 rows) or 16-row tiles that share one
@@ -291,11 +297,26 @@ constexpr size_t kBlockBytes = 74 * 1024 + 256;  // shared memory of a block of 
 constexpr int kMinKeys = 128;    // a block's keys before the next block is used
 constexpr int kMaxStages = 4;
 constexpr int kFlushKeys = 512;  // keys whose products a warp leaves to the tensor core's own sums
+// P is 2^kHead at most when a row's reference is set and 2^(kHead + kRise) before it is
+// moved; with scales below 2^kTop, P * scale is below 2^15.  With this kTop the factors of
+// scales from 2^-23 to 2^16 are f16 numbers.  24 x 8 heads of up to 32K keys, and 16 x 8 of up
+// to 4K with 40 rows: 153 and 100 us with kRise 5; 153 and 99 with 8, which leaves three bits
+// less below the largest; 154 and 102 with 3.  A factor for the block's scales costs 1 to 2 us
+// of these, and 1.4 of 57 in a tracked decode step.
+constexpr int kTop = -8;
+constexpr float kHead = 18.0f, kRise = 5.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The warp's largest |x|.
+__device__ __forceinline__ float warp_absmax(float x) {
+  float y;
+  asm("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -650,6 +671,44 @@ __device__ __forceinline__ void load_scales(const float* p, f32x2 (&s)[NB]) {
 template <int NB, int KEYS>
 constexpr int stage_bytes() { return KEYS * NB * 36; }
 
+// The f16 scales of 32 keys, as a lane reads them from a stage: key pairs and one
+// or two blocks, keys' before values'.
+template <int NB>
+struct RawScales {
+  static constexpr int kPer = NB % 2 ? 1 : 2;  // blocks of an item
+  static constexpr int kItems = kStep / 2 * NB / kPer, kRounds = (2 * kItems + 31) / 32;
+  uint32_t w[kRounds][2];  // of the pair's two keys: kPer halves each
+};
+
+// The powers of two that a warp's value scales are multiplied by, one a block.
+template <int NB>
+struct ValueFactors {
+  unsigned fields;  // byte b: the exponent field of block b's
+  uint32_t lane;    // f16, of the value scales that this lane converts (1 for key scales): of a round's two blocks, or of two rounds
+  static constexpr int kLargest = 127 + 15, kSmallest = 127 - 24;  // f16's powers of two
+
+  __device__ __forceinline__ float of(int b) const { return __uint_as_float((fields >> (8 * b) & 0xFFu) << 23); }
+  __device__ __forceinline__ float inverse(int b) const { return __uint_as_float((254u - (fields >> (8 * b) & 0xFFu)) << 23); }
+  __device__ __forceinline__ void set_lane() {
+    using S = RawScales<NB>;
+    const int i0 = 32 * (S::kRounds - (NB == 3 ? 2 : 1)) + (threadIdx.x & 31), i1 = NB == 3 ? i0 + 32 : i0;
+    auto factor = [&](int i, int more) { return i < S::kItems ? 1.0f : of((i - S::kItems) % (NB / S::kPer) * S::kPer + more); };
+    lane = pack_half2(factor(i0, 0), factor(i1, S::kPer - 1));
+  }
+  __device__ __forceinline__ void init() {
+    fields = 0x01010101u * kLargest;
+    set_lane();
+  }
+};
+// x's half `high` times f's, exactly, in f32.
+__device__ __forceinline__ float mul_halves(uint32_t x, int high, uint32_t f, int high_f) {
+  float y;
+  asm("{\n\t.reg .b16 a, b;\n\tcvt.u16.u32 a, %1;\n\tcvt.u16.u32 b, %2;\n\tfma.rn.f32.f16 %0, a, b, %3;\n\t}"
+      : "=f"(y)
+      : "r"(high ? x >> 16 : x), "r"(high_f ? f >> 16 : f), "f"(0.0f));
+  return y;
+}
+
 // What a warp carries over its keys for its rows (lane: rows g and g + 8, columns by t).
 template <int NB, int R>
 struct RowState {
@@ -658,16 +717,7 @@ struct RowState {
   float m[R];    // running maximum that the reference was set from (row)
   float ref[R];  // reference: P = exp2(score - ref)
   f32x2 l[R];    // sums of P over the lane's even and odd keys
-  int lim;       // 2^lim bounds the value scales seen (warp)
-};
-
-// The f16 scales of 32 keys, as a lane reads them from a stage: key pairs and one
-// or two blocks, keys' before values'.
-template <int NB>
-struct RawScales {
-  static constexpr int kPer = NB % 2 ? 1 : 2;  // blocks of an item
-  static constexpr int kItems = kStep / 2 * NB / kPer, kRounds = (2 * kItems + 31) / 32;
-  uint32_t w[kRounds][2];  // of the pair's two keys: kPer halves each
+  ValueFactors<NB> scaled;  // of the value scales; the sums count by them too
 };
 
 // ks, vs: the key and value scales of the 32 keys.
@@ -691,10 +741,11 @@ __device__ __forceinline__ RawScales<NB> load_raw_scales(const uint8_t* ks, cons
 }
 
 // The same as float32 [key pair][block][2], keys' first and then values', in shared
-// memory: each is needed by 8 lanes, and is converted once.  Keys from len on
-// (whatever they hold) become 0.  Returns the lane's largest value scale.
+// memory: each is needed by 8 lanes, and is converted once.  Value scales are multiplied by
+// the factors f of their blocks.  Keys from len on (whatever they hold) become 0.
+// Returns the lane's largest value scale after that.
 template <int NB, bool MASKED>
-__device__ __forceinline__ float convert_scales(const RawScales<NB>& raw, float* to, int k0, int len) {
+__device__ __forceinline__ float convert_scales(const RawScales<NB>& raw, float* to, int k0, int len, uint32_t f) {
   using R = RawScales<NB>;
   const int lane = threadIdx.x & 31;
   float dmax = 0.0f;
@@ -708,7 +759,10 @@ __device__ __forceinline__ float convert_scales(const RawScales<NB>& raw, float*
     float2 x[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      x[c] = unpack_half2(raw.w[n][c]);
+      if (32 * n + 31 < R::kItems)  // key scales alone
+        x[c] = unpack_half2(raw.w[n][c]);
+      else
+        x[c] = make_float2(mul_halves(raw.w[n][c], 0, f, NB == 3 ? n - 1 : 0), R::kPer == 2 ? mul_halves(raw.w[n][c], 1, f, 1) : 0.0f);
       if (MASKED && k0 + 2 * pair + c >= len) x[c] = make_float2(0.0f, 0.0f);
       if (value) dmax = fmaxf(dmax, R::kPer == 2 ? fmaxf(fabsf(x[c].x), fabsf(x[c].y)) : fabsf(x[c].x));
     }
@@ -721,14 +775,82 @@ __device__ __forceinline__ float convert_scales(const RawScales<NB>& raw, float*
   return dmax;
 }
 
+// The tensor core cuts its sums off instead of rounding them, which is a drift over
+// a long run of keys: results 1.3e-6 off after 2048 keys of one warp.  So a warp
+// adds its sums to float32 ones, rounded, every kFlushKeys keys (8 rows; 16 rows, of
+// twice the products a key, every half of that): 2e-7 and 8e-7 off.  These lie in
+// local memory (`volatile`): the loop has no registers for them.  24 x 8 heads of up
+// to 32K keys: 152 us, 151 every 1024 keys (2.7e-7).  They are relative to the
+// reference of their time.
+template <int NB, int R>
+struct FlushedSums {
+  volatile float o[NB * 8 * R];
+  float ref[R];  // -inf: no key was seen (the sums are 0 or NaN); +inf: nothing was flushed
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < R; ++i) ref[i] = INFINITY;
+  }
+  __device__ __forceinline__ bool any() const { return ref[0] != INFINITY; }
+  // Column c (0, 1) of the lane's row i, from the warp's sums.
+  static __device__ __forceinline__ float sum(const RowState<NB, R>& r, int n, int i, int c) {
+    return R == 1 ? __fsub_rn(r.o[n][c], r.o[n][2 + c]) : r.o[n][2 * i + c];
+  }
+  __device__ __forceinline__ float total(const RowState<NB, R>& r, int n, int i, int c) const {
+    return any() ? o[(n * R + i) * 2 + c] : sum(r, n, i, c);
+  }
+  // The sums of a block whose value scales are divided by 2^less (byte b: block b).
+  __device__ __forceinline__ void scale(unsigned less) {
+#pragma unroll 1
+    for (int n = 0; n < NB * 8 * R; ++n) o[n] = __fmul_rn(o[n], __uint_as_float((127u - (less >> (n / R & ~7) & 0xFFu)) << 23));
+  }
+  __device__ __forceinline__ void flush(RowState<NB, R>& r) {
+    const bool add = any();
+    float f[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      f[i] = ref[i] == r.ref[i] ? 1.0f : exp2_fast(ref[i] - r.ref[i]);
+      ref[i] = r.m[i] == -INFINITY ? -INFINITY : r.ref[i];
+    }
+    constexpr int kRun = R == 1 ? NB * 4 : 4;  // all loads of a run before its first store
+#pragma unroll
+    for (int n0 = 0; n0 < NB * 4; n0 += kRun) {
+      float old[kRun][R][2];
+#pragma unroll
+      for (int n = 0; n < kRun; ++n)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            old[n][i][c] = 0.0f;
+            if (add) old[n][i][c] = o[((n0 + n) * R + i) * 2 + c];
+          }
+#pragma unroll
+      for (int n = 0; n < kRun; ++n)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = sum(r, n0 + n, i, c);
+            o[((n0 + n) * R + i) * 2 + c] = add ? __fmaf_rn(old[n][i][c], f[i], x) : x;
+          }
+    }
+#pragma unroll
+    for (int n = 0; n < NB * 4; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) r.o[n][x] = 0.0f;
+  }
+};
+
 // 32 keys from k0 on: kc and vc their key and value codes, scales where their
 // converted scales go.  row_end: keys before it are seen by the lane's rows; MASKED:
 // some key is not, for some row.
 template <int NB, int R, bool MASKED>
 __device__ __forceinline__ void keys32(const uint8_t* kc, const uint8_t* vc, const RawScales<NB>& raw, float* scales, int k0,
-                                       int len, const int (&row_end)[R], const WarpQueries<NB, R>& q, RowState<NB, R>& r) {
+                                       int len, const int (&row_end)[R], const WarpQueries<NB, R>& q, RowState<NB, R>& r,
+                                       FlushedSums<NB, R>& flushed) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const float dmax = convert_scales<NB, MASKED>(raw, scales, k0, len);
+  const float dmax = convert_scales<NB, MASKED>(raw, scales, k0, len, r.scaled.lane);
   __syncwarp();
   f32x2 z[4][R];  // keys 8 j + 2t, + 1
   if constexpr (WarpQueries<NB, R>::kShared) {
@@ -773,7 +895,8 @@ __device__ __forceinline__ void keys32(const uint8_t* kc, const uint8_t* vc, con
       }
   }
   float zmax[R];
-  bool moves = dmax >= __int_as_float((r.lim + 127) << 23);
+  constexpr float kTopScale = 1.0f / (1 << -kTop);
+  bool moves = dmax >= kTopScale;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     zmax[i] = -INFINITY;
@@ -782,19 +905,38 @@ __device__ __forceinline__ void keys32(const uint8_t* kc, const uint8_t* vc, con
       const float2 v = unpair2(z[j][i]);
       zmax[i] = fmaxf(zmax[i], fmaxf(v.x, v.y));
     }
-    moves = moves || zmax[i] > r.m[i] + 8.0f;
+    moves = moves || zmax[i] > r.m[i] + kRise;
   }
   if (__any_sync(0xffffffffu, moves)) {
-    const float dm = mri::warp_max(dmax);
-    // dm < 2^lim (the largest finite scale is 65504; an infinite one spoils its own sums only).
-    r.lim = max(r.lim, min(16, static_cast<int>(__float_as_uint(dm) >> 23) - 126));
+    float by[NB];
+    unsigned less = 0;  // byte b: by how many powers of two
+    if (__any_sync(0xffffffffu, dmax >= kTopScale)) {
+      // A block with such a scale takes a smaller factor, and so do its sums.  An infinite
+      // scale does not count: it spoils the sums of rows that see it, and no others.
+      float* s = scales + kStep * NB + (lane >> 1) * (2 * NB) + (lane & 1);
+#pragma unroll 1
+      for (int b = 0; b < NB; ++b) {
+        const float x = s[2 * b];
+        const float top = warp_absmax(fabsf(x) < INFINITY ? x : 0.0f);
+        const int over = static_cast<int>(__float_as_uint(top) >> 23) - (127 + kTop - 1);
+        const int n = max(0, min(over, static_cast<int>(r.scaled.fields >> (8 * b) & 0xFFu) - ValueFactors<NB>::kSmallest));
+        less |= static_cast<unsigned>(n) << (8 * b);
+        s[2 * b] = __fmul_rn(x, __uint_as_float(static_cast<unsigned>(127 - n) << 23));
+      }
+      r.scaled.fields -= less;
+      if (flushed.any()) flushed.scale(less);
+      r.scaled.set_lane();
+      __syncwarp();
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) by[b] = __uint_as_float((127u - (less >> (8 * b) & 0xFFu)) << 23);
     float f[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float mn = fmaxf(zmax[i], __shfl_xor_sync(0xffffffffu, zmax[i], 1));
       mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
-      mn = mn > r.m[i] + 8.0f ? mn : r.m[i];  // a row moves on its own scores only
-      const float ref = mn == -INFINITY ? 0.0f : mn + static_cast<float>(r.lim - 6);
+      mn = mn > r.m[i] + kRise ? mn : r.m[i];  // a row moves on its own scores only
+      const float ref = mn == -INFINITY ? 0.0f : mn - kHead;
       f[i] = r.m[i] == -INFINITY ? 0.0f : exp2_fast(r.ref[i] - ref);
       r.m[i] = mn;
       r.ref[i] = ref;
@@ -803,7 +945,7 @@ __device__ __forceinline__ void keys32(const uint8_t* kc, const uint8_t* vc, con
 #pragma unroll
     for (int n = 0; n < NB * 4; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) r.o[n][x] = __fmul_rn(r.o[n][x], f[R == 1 ? 0 : x / 2]);
+      for (int x = 0; x < 4; ++x) r.o[n][x] = __fmul_rn(r.o[n][x], __fmul_rn(f[R == 1 ? 0 : x / 2], by[n / 4]));
   }
   f32x2 nref[R];
 #pragma unroll
@@ -881,77 +1023,15 @@ __device__ __forceinline__ void keys32(const uint8_t* kc, const uint8_t* vc, con
   }
 }
 
-// The tensor core cuts its sums off instead of rounding them, which is a drift over
-// a long run of keys: results 1.3e-6 off after 2048 keys of one warp.  So a warp
-// adds its sums to float32 ones, rounded, every kFlushKeys keys (8 rows; 16 rows, of
-// twice the products a key, every half of that): 2e-7 and 8e-7 off.  These lie in
-// local memory (`volatile`): the loop has no registers for them.  24 x 8 heads of up
-// to 32K keys: 152 us, 151 every 1024 keys (2.7e-7).  They are relative to the
-// reference of their time.
-template <int NB, int R>
-struct FlushedSums {
-  volatile float o[NB * 8 * R];
-  float ref[R];  // -inf: no key was seen (the sums are 0 or NaN); +inf: nothing was flushed
-
-  __device__ __forceinline__ void init() {
-#pragma unroll
-    for (int i = 0; i < R; ++i) ref[i] = INFINITY;
-  }
-  __device__ __forceinline__ bool any() const { return ref[0] != INFINITY; }
-  // Column c (0, 1) of the lane's row i, from the warp's sums.
-  static __device__ __forceinline__ float sum(const RowState<NB, R>& r, int n, int i, int c) {
-    return R == 1 ? __fsub_rn(r.o[n][c], r.o[n][2 + c]) : r.o[n][2 * i + c];
-  }
-  __device__ __forceinline__ float total(const RowState<NB, R>& r, int n, int i, int c) const {
-    return any() ? o[(n * R + i) * 2 + c] : sum(r, n, i, c);
-  }
-  __device__ __forceinline__ void flush(RowState<NB, R>& r) {
-    const bool add = any();
-    float f[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      f[i] = ref[i] == r.ref[i] ? 1.0f : exp2_fast(ref[i] - r.ref[i]);
-      ref[i] = r.m[i] == -INFINITY ? -INFINITY : r.ref[i];
-    }
-    constexpr int kRun = R == 1 ? NB * 4 : 4;  // all loads of a run before its first store
-#pragma unroll
-    for (int n0 = 0; n0 < NB * 4; n0 += kRun) {
-      float old[kRun][R][2];
-#pragma unroll
-      for (int n = 0; n < kRun; ++n)
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            old[n][i][c] = 0.0f;
-            if (add) old[n][i][c] = o[((n0 + n) * R + i) * 2 + c];
-          }
-#pragma unroll
-      for (int n = 0; n < kRun; ++n)
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float x = sum(r, n0 + n, i, c);
-            o[((n0 + n) * R + i) * 2 + c] = add ? __fmaf_rn(old[n][i][c], f[i], x) : x;
-          }
-    }
-#pragma unroll
-    for (int n = 0; n < NB * 4; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) r.o[n][x] = 0.0f;
-  }
-};
-
 // One stage, 32 keys at a time.
 template <int NB, int R, int KEYS, bool MASKED>
 __device__ __forceinline__ void stage_keys(const uint8_t* st, float* scales, int k0, int len, const int (&row_end)[R],
-                                           const WarpQueries<NB, R>& q, RowState<NB, R>& r) {
+                                           const WarpQueries<NB, R>& q, RowState<NB, R>& r, FlushedSums<NB, R>& flushed) {
 #pragma unroll 1
   for (int h = 0; h < KEYS; h += kStep) {
     if (KEYS > kStep) __syncwarp();  // the scales of the step before are read
     const RawScales<NB> raw = load_raw_scales<NB>(st + KEYS * NB * 32 + h * (2 * NB), st + KEYS * NB * 34 + h * (2 * NB));
-    keys32<NB, R, MASKED>(st + h * (16 * NB), st + (KEYS + h) * (16 * NB), raw, scales, k0 + h, len, row_end, q, r);
+    keys32<NB, R, MASKED>(st + h * (16 * NB), st + (KEYS + h) * (16 * NB), raw, scales, k0 + h, len, row_end, q, r, flushed);
   }
 }
 
@@ -1175,7 +1255,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
       r.ref[i] = 0.0f;
       r.l[i] = 0;
     }
-    r.lim = -24;
+    r.scaled.init();
     FlushedSums<NB, R> flushed;
     flushed.init();
 #pragma unroll
@@ -1190,9 +1270,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
       if (!dead) {
         const int k0 = (y - unit_begin) * KEYS;
         if (k0 + KEYS > clear)
-          stage_keys<NB, R, KEYS, true>(ring + s * SB, scales_sh, k0, len, row_end, q, r);
+          stage_keys<NB, R, KEYS, true>(ring + s * SB, scales_sh, k0, len, row_end, q, r, flushed);
         else
-          stage_keys<NB, R, KEYS, false>(ring + s * SB, scales_sh, k0, len, row_end, q, r);
+          stage_keys<NB, R, KEYS, false>(ring + s * SB, scales_sh, k0, len, row_end, q, r, flushed);
       }
       __syncwarp();
       if (a.row_tiles > 1 && lane == 0) mri::mbar_arrive(&emptyw[s]);
@@ -1227,11 +1307,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs 
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {  // odd places of each four were 16-fold
+          const float unit = r.scaled.inverse(b), part = __fmul_rn(unit, 0.0625f);
           float4 v;
-          v.x = flushed.total(r, 4 * b, i, c);
-          v.y = __fmul_rn(flushed.total(r, 4 * b + 1, i, c), 0.0625f);
-          v.z = flushed.total(r, 4 * b + 2, i, c);
-          v.w = __fmul_rn(flushed.total(r, 4 * b + 3, i, c), 0.0625f);
+          v.x = __fmul_rn(flushed.total(r, 4 * b, i, c), unit);
+          v.y = __fmul_rn(flushed.total(r, 4 * b + 1, i, c), part);
+          v.z = __fmul_rn(flushed.total(r, 4 * b + 2, i, c), unit);
+          v.w = __fmul_rn(flushed.total(r, 4 * b + 3, i, c), part);
           const int col = 32 * b + 8 * t + 4 * c;
           if (R == 1)
             *reinterpret_cast<float4*>(mine + col) = v;
