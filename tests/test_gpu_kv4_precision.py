@@ -110,3 +110,31 @@ def test_infinite_value_scale_that_rows_do_not_see(mri, gpu_ctx, group):
     assert np.array_equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("tokens,group", [(1, 2), (5, 2)])
+def test_sums_over_many_keys_of_a_warp(mri, gpu_ctx, tokens, group):
+    """So many keys that a warp walks some 19000 of one head.  Sums that the tensor core cuts
+    off drift by half a unit a step, 1200 steps of 16 keys; added to rounded ones every 512
+    keys (8 rows: high and low parts have sums of their own) or 256 (16 rows: both in one)
+    they are 32 cuts from that.  Without it both are off by more than the bound."""
+    import torch
+    heads, d, cap = 128, 128, 262144
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    cache = mri.KVCache4(1, heads, d, cap)
+    # Value codes 8 to 15: values of one sign, so that a drift shows whole.
+    cache.k.random_(0, 256, generator=gen)
+    cache.v.random_(0, 256, generator=gen).bitwise_or_(0x88)
+    cache.k_scale.fill_(0.25)
+    cache.v_scale.copy_(torch.rand(cache.v_scale.shape, generator=gen, device="cuda") * 0.1 + 0.2)
+    q = torch.randn(1, tokens, heads * group, d, generator=gen, device="cuda") * 0.02
+    got = cache.attention(q, i32([cap]))
+    for head in (0, 61, 127):
+        one = mri.KVCache4.from_tensors(*(t[:, head:head + 1].contiguous() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weight)))
+        k, v = (t[0, :, 0].double() for t in one.read(None, cap))
+        for t in range(tokens):
+            seen = cap - tokens + 1 + t
+            for g in range(group):
+                row = q[0, t, head * group + g].double()
+                a = float((k[:seen].abs() @ row.abs()).max()) * d ** -0.5
+                want = torch.softmax(k[:seen] @ row * d ** -0.5, 0) @ v[:seen]
+                err = ((got[0, t, head * group + g].double() - want).abs() / want).max()
+                assert float(err) <= (24 * a + 32 + 32) * 2.0 ** -23, (head, t, g, float(err), a)
