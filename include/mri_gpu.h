@@ -406,9 +406,10 @@ MRI_API int mri_kv4_evict(mri_ctx* ctx, const mri_kv4_cache* src, const int32_t*
 /* ── verification of drafted tokens ────────────────────────────────────────── */
 /* No counterpart in the reference.  Speculative sampling: n_drafts tokens were
  * drafted for each of `batch` sequences, the model gave logits for the positions
- * of all of them and one more (mri_llama_forward_at on the draft).
- *   target_logits [batch][n_drafts + 1][vocab] f32; NaN counts as -inf, +inf as
- *     the largest finite value
+ * of all of them and one more.
+ *   target_logits [batch][n_drafts + 1][vocab] f32, in device memory (what
+ *     mri_llama_forward_at gives is host memory and has to be copied); NaN counts as
+ *     -inf, +inf as the largest finite value
  *   draft_tokens  [batch][n_drafts] int32; one outside [0, vocab) is rejected
  *   draft_probs   [batch][n_drafts][vocab] f32, the distributions they were
  *     sampled from; null when they were chosen, not sampled (probability 1)

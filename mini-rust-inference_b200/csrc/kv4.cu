@@ -217,8 +217,9 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(Cache c, const flo
   }
 }
 
-// Bound by HBM (d + 4 NB bytes read, 8 d written a row): 128000 rows of 128 in 36.5 us,
-// 4.1 TB/s.  Two rows a thread were slower: the writes are what it waits for.
+// Bound by the writes (d + 4 NB bytes read, 8 d written a row): 128000 rows of 128 in 36 us,
+// 4.1 TB/s.  Each of a thread's two 16-byte writes is half a sector, and a warp's cover 1 KB
+// by halves.  Two rows a thread were slower.
 template <int NB>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, const int32_t* __restrict__ start,
                                                             unsigned n_tokens, float* __restrict__ k,
@@ -780,7 +781,7 @@ __device__ __forceinline__ float convert_scales(const RawScales<NB>& raw, float*
 // adds its sums to float32 ones, rounded, every kFlushKeys keys (8 rows; 16 rows, of
 // twice the products a key, every half of that): 2e-7 and 8e-7 off.  These lie in
 // local memory (`volatile`): the loop has no registers for them.  24 x 8 heads of up
-// to 32K keys: 152 us, 151 every 1024 keys (2.7e-7).  They are relative to the
+// to 32K keys: 153 us, 1 less every 1024 keys (2.7e-7).  They are relative to the
 // reference of their time.
 template <int NB, int R>
 struct FlushedSums {
@@ -1151,8 +1152,8 @@ __device__ __forceinline__ float* part_at(const AttnArgs& a, int cta, int c0) {
 // and a kernel of its own merges what several blocks had a part in (the last block
 // alone took 30K clocks for 40 rows of 128).
 // Bound by instruction issue at three warps of 168 registers a scheduler.  24 x 8 heads
-// of up to 32K keys, 8 rows of 128: 152 us, 3.0 TB/s, 53 % of issue slots.  16 x 8
-// heads of up to 4K keys, 40 rows: 80 us (all 8 rows a warp: 107).  2 x 32 heads of 64,
+// of up to 32K keys, 8 rows of 128: 153 us, 3.0 TB/s, 53 % of issue slots.  16 x 8
+// heads of up to 4K keys, 40 rows: 82 us (all 8 rows a warp: 107).  2 x 32 heads of 64,
 // 509 rows: 111 us (8 rows a warp: 159).
 template <int NB, int R>
 __global__ void __launch_bounds__(kMaxWarps * 32, 3) kv4_attend_kernel(AttnArgs a) {

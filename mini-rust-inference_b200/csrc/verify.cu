@@ -156,12 +156,15 @@ __device__ __forceinline__ void put_remote(const void* p, int rank, int4 v) {
 // summed; a warp's maxima and sums stay with it until all rows are read.  The blocks
 // tell each other their rows' statistics, each merges them and decides how many
 // drafts stand, and scores its part of the next token's row, which is in L2 by
-// then; the first block takes the best of all.  Exponentials are the 2-ulp ones (the
-// acceptance test uses expf).  Bound by instruction issue and HBM for a batch (256
-// sequences of 5 rows of 32000: 48 us, 3.5 TB/s), by latency for one sequence (5 rows
-// of 32000: 8 us): a round trip a row, two cluster barriers, the second row's loads.
-// Two kernels with a block for each 1024 or 4096 values of a row took 74 and 7.7 us on
-// the GPU, but the host 2.5 us more a call, which is what a lone call waits for.
+// then; the first block takes the best of all.  Exponentials of the rows are ex2.approx of
+// an argument rounded to f32: 2 units in the last place near p = 1, some 20 at p =
+// e^-20 (the acceptance test and the merges use expf).  Bound by instruction issue and HBM
+// for a batch (256 sequences of 5 rows of 32000: 48 us, 3.5 TB/s), by latency for one
+// sequence (5 rows of 32000: 8.5 us): a round trip a row, two cluster barriers, the second
+// row's loads.  Two kernels with a block for each 1024 or 4096 values of a row took 74 us
+// for the 256 sequences, but 7.7 for the one, and 12.5 for 16 of 4 rows of 50001 where this
+// takes 17; against that stand 2.5 us a call of the host, which is what a lone call waits
+// for (and which a CUDA graph does not pay).
 template <int PER, bool VEC>
 __global__ void __launch_bounds__(PER == kPerMany ? kManyThreads : kFewThreads, PER == kPerMany ? 4 : 2) verify_kernel(Args a) {
   __shared__ Stat sh_warp[kMaxDrafts + 1][kMaxWarps];       // of this block's warps
@@ -407,7 +410,7 @@ extern "C" int mri_verify_draft(mri_ctx* ctx, const float* target_logits_dev, co
   }
   // Blocks of a sequence: as many as the GPU still takes at once, each with at least
   // 2048 values of a row.  48 sequences of 8 rows of 32000: 21 us with 16 values a
-  // thread, 31 with 8; one of 5 rows: 9.0 and 8.2; 16 of 4 rows of 50001: 17 us in
+  // thread, 31 with 8; one of 5 rows: 9.0 and 8.2 to 8.5; 16 of 4 rows of 50001: 17 us in
   // blocks of up to 512 threads, 23 of up to 1024 (not all clusters run at once).
   const size_t sms = static_cast<size_t>(ctx->dev.sm_count);
   size_t blocks = kMaxCluster;
